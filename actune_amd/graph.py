@@ -2,12 +2,13 @@
 
 Same contract as actune/graph.py:6-95. One hipGraph (torch.cuda.CUDAGraph on
 ROCm) is captured per (argument tree, tensor shapes/strides/dtypes/devices,
-non-tensor reprs, every layer's active mode), up to ``max_graphs``; beyond
-that calls run eagerly and are counted as fallbacks. Capture warms the
+non-tensor reprs, every layer's active mode, the active adapter scope's ids as
+one more tensor or none), up to ``max_graphs``; beyond that calls run eagerly
+and are counted as fallbacks. Capture warms the
 function twice on a side stream, records the per-layer ``calls`` /
 ``input_elements`` seen during capture and restores the live counters;
-each replay copies the inputs into the captured static buffers, replays and
-adds the recorded counts, so BankRuntime.audit sees the same numbers as
+each replay copies the inputs (the adapter scope's ids among them) into the
+captured static buffers, replays and adds the recorded counts, so BankRuntime.audit sees the same numbers as
 eager execution. The returned output is graph-owned (overwritten by the next
 replay of the same graph).
 
@@ -24,6 +25,7 @@ from unittest.mock import patch
 import torch
 from torch.utils import _pytree as pytree
 
+from .kernels.adapters import active_adapter_ids, adapter_scope
 from .precision import active_precision_profile
 
 
@@ -79,7 +81,7 @@ class GraphReplay:
 
     def _key(self, leaves, spec):
         sig = []
-        for leaf in leaves:
+        for leaf in (*leaves, active_adapter_ids()):
             if isinstance(leaf, torch.Tensor):
                 sig.append((tuple(leaf.shape), tuple(leaf.stride()), str(leaf.dtype), str(leaf.device)))
             else:
@@ -90,14 +92,14 @@ class GraphReplay:
 
     def _capture(self, leaves, spec):
         saved = {name: (m.calls, m.input_elements) for name, m in self.layers.items()}
-        static = [x.clone() if isinstance(x, torch.Tensor) else x for x in leaves]
-        args, kwargs = pytree.tree_unflatten(static, spec)
+        static = [x.clone() if isinstance(x, torch.Tensor) else x for x in (*leaves, active_adapter_ids())]
+        args, kwargs = pytree.tree_unflatten(static[:-1], spec)
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         # the first warm-up pass records which group-64 inputs several
         # linears share; the second pass and the capture follow that plan
         plan = None
-        with torch.cuda.stream(side), torch.inference_mode():
+        with torch.cuda.stream(side), torch.inference_mode(), adapter_scope(static[-1]):
             for _ in range(2):
                 with self.scope(plan) as group_codes:
                     self.function(*args, **kwargs)
@@ -107,7 +109,7 @@ class GraphReplay:
         for m in self.layers.values():
             m.calls = m.input_elements = 0
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph), torch.inference_mode(), self.scope(plan):
+        with torch.cuda.graph(graph), torch.inference_mode(), adapter_scope(static[-1]), self.scope(plan):
             output = self.function(*args, **kwargs)
         self.sharing_plans[self._key(leaves, spec)] = plan
         counts = {name: (m.calls, m.input_elements) for name, m in self.layers.items()}
@@ -127,7 +129,7 @@ class GraphReplay:
                 return self.function(*args, **kwargs)
             entry = self.graphs[key] = self._capture(leaves, spec)
         graph, static, output, counts = entry
-        for src, dst in zip(leaves, static, strict=True):
+        for src, dst in zip((*leaves, active_adapter_ids()), static, strict=True):
             if isinstance(src, torch.Tensor):
                 dst.copy_(src)
         graph.replay()

@@ -78,13 +78,21 @@ def adapter_add(y, x, a, b, scaling, ids, out=None):
 def adapter_scope(ids):
     """The adapter of each request (int32, leading dimensions of the linears'
     inputs; None: no adapters) for the AdaptedLinears of one forward. The
-    tensor is read when the launches run: under GraphReplay make it an
-    argument of the captured function, so that a replay reads its values."""
+    tensor is read when the launches run. Around a GraphReplay it is an input
+    like the call's arguments: a graph belongs to a scope's shape of ids (or to
+    none), and a replay reads the values that the scope has then. A scope
+    inside the captured function reads the tensor that it was captured with:
+    make that one an argument of the function."""
     token = _IDS.set(ids)
     try:
         yield
     finally:
         _IDS.reset(token)
+
+
+def active_adapter_ids():
+    """The ids of the innermost adapter_scope (None: no adapters)."""
+    return _IDS.get()
 
 
 class AdaptedLinear(torch.nn.Module):
@@ -109,7 +117,7 @@ class AdaptedLinear(torch.nn.Module):
     def adapt(self, y, x):
         """y (the linear's output on x, which this may write) with the scope's
         adapters added: for outputs of a call that runs several linears."""
-        ids = _IDS.get()
+        ids = active_adapter_ids()
         if ids is None:
             return y
         return adapter_add(y, x, self.a, self.b, self.scaling, ids, out=y if y.is_contiguous() else None)
