@@ -125,6 +125,27 @@ def fast():
     return _FAST
 
 
+# what drops the codes that it holds of a tensor, given a tensor that has been written
+_ON_WRITE = []
+
+
+def written(tensor) -> None:
+    """Says that a kernel wrote a caller's tensor in place, as torch's own
+    in-place operators say it: the version counter moves, so that codes held of
+    the old values are not taken for the new ones. Inference tensors have no
+    counter: the caches drop what they hold of that memory."""
+    if not tensor.is_inference():
+        torch.autograd.graph.increment_version(tensor)
+        return
+    for forget in _ON_WRITE:
+        forget(tensor)
+
+
+def same_memory(a, b) -> bool:
+    """Whether two tensors are views of one allocation."""
+    return a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr()
+
+
 def _check(rc: int) -> None:
     if rc:
         msg = lib().actune_last_error().decode()

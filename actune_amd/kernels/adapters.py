@@ -28,11 +28,14 @@ def adapter_add(y, x, a, b, scaling, ids, out=None):
     for each row or, with fewer dimensions, for each of the leading ones ([B]
     for x [B, T, K]). A row whose id is not in [0, L) (-1, say) keeps y.
     1 <= R <= 128; adapters of a lower rank are padded with zeros. out: a
-    tensor to write to, y itself included; a new one by default. Sums in f32,
-    one rounding at the end.
+    tensor to write to, y itself included; a new one by default (written as by
+    torch's in-place operators: codes that a shared scope holds of it are not
+    used again). Sums in f32, one rounding at the end.
     """
     done = _block.fast().adapter_add(y, x, a, b, scaling, ids, out)
     if done is not None:
+        if out is not None:
+            _native.written(out)
         return done
     _block.check_inputs([("x", x), ("y", y), ("a", a), ("b", b)] + ([] if out is None else [("out", out)]), _TYPES)
     if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
@@ -61,7 +64,8 @@ def adapter_add(y, x, a, b, scaling, ids, out=None):
     need = _block.lib().actune_adapter_workspace_bytes(m, n, k, rank)
     if need < 0:
         raise ValueError("invalid dimensions")
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty(y.shape, dtype=y.dtype, device=y.device)
     work = torch.empty(need, dtype=torch.uint8, device=x.device)
     args = _block.AdapterArgs(
@@ -71,6 +75,8 @@ def adapter_add(y, x, a, b, scaling, ids, out=None):
         ids_rows=m // ids.numel() if m and ids.numel() else 1, M=m, N=n, K=k, R=rank, L=count,
         dtype=_native.DTYPE_CODES[x.dtype])
     _block.launch("actune_adapter_add", args, x.device)
+    if given:
+        _native.written(out)
     return out
 
 

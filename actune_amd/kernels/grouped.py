@@ -123,6 +123,15 @@ def _shared_codes(state, source, flat, a, input_scale):
     return packed, scales
 
 
+def _forget_codes(tensor):
+    state = _SHARED_GROUP_STATE.get()
+    if state is not None and state.entries and _native.same_memory(state.entries[0][0], tensor):
+        state.entries.clear()
+
+
+_native._ON_WRITE.append(_forget_codes)
+
+
 def extension():
     """The native op object (reference: the JIT extension, grouped.py:97-105)."""
     return _native.extension()

@@ -346,6 +346,17 @@ def clear_shared_a8_cache() -> None:
     state.entry = state.a4_entry = None
 
 
+def _forget_codes(tensor):
+    state = _SHARED_A8.get()
+    for slot in ("entry", "a4_entry"):
+        held = getattr(state, slot, None)
+        if held is not None and _native.same_memory(held.source, tensor):
+            setattr(state, slot, None)
+
+
+_native._ON_WRITE.append(_forget_codes)
+
+
 @contextmanager
 def shared_a8_cache_scope(*, enabled: bool = True) -> Iterator[SharedA8CacheStats]:
     """A fresh cache for the body (one model forward); its codes are dropped

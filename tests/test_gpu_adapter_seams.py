@@ -1,11 +1,13 @@
 """The adapters where they meet the rest of the framework, on the GPU: graph
-replay under an adapter scope."""
+replay under an adapter scope, codes that linears share."""
 import pytest
 import torch
 
+from actune_amd import _block, _native
 from actune_amd.graph import GraphReplay
-from actune_amd.kernels.adapters import AdaptedLinear, adapter_scope
-from actune_amd.kernels.grouped import GroupedPaddedLinear
+from actune_amd.kernels.adapters import AdaptedLinear, adapter_add, adapter_scope
+from actune_amd.kernels.grouped import GroupedPaddedLinear, shared_activation_scope
+from actune_amd.kernels.tokenwise import W4A8TritonLinear, shared_a8_cache_scope
 
 pytestmark = pytest.mark.gpu
 
@@ -56,3 +58,38 @@ def test_replays_follow_the_adapter_scope():
         assert torch.equal(each[0, 0], alone[0, 0]) and not torch.equal(each, second)
         assert torch.equal(check(None), alone)
         assert len(replay.graphs) == 3 and replay.replays == 15 and replay.fallbacks == 0
+
+
+@pytest.mark.parametrize("mode", [torch.inference_mode, torch.no_grad, torch.enable_grad])
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("kind", ["groups", "rows"])
+def test_codes_of_a_written_tensor_are_not_used_again(mode, native, kind, monkeypatch):
+    """lin(t), adapters added to t in place, lin2(t) in one scope of shared codes: lin2 reads what t holds then, also where
+    the call wrote through a view; codes of a tensor that was not written are still shared."""
+    if not native:
+        monkeypatch.setattr(_block, "_FAST", _native._CtypesOnly())
+    torch.manual_seed(1)
+    with torch.no_grad():
+        if kind == "groups":
+            scope, (first, second) = shared_activation_scope, (_packed(512, 512), _packed(512, 128))
+        else:
+            scope = shared_a8_cache_scope
+            first, second = (W4A8TritonLinear(torch.nn.Linear(512, n, dtype=torch.bfloat16, device=DEV)) for n in (512, 128))
+    with mode():
+        x, t = (torch.randn(48, 512, device=DEV, dtype=torch.bfloat16) for _ in range(2))
+        a = torch.randn(2, 8, 512, device=DEV, dtype=torch.bfloat16)
+        b = torch.randn(2, 512, 8, device=DEV, dtype=torch.bfloat16)
+        scaling, ids = torch.ones(2, device=DEV), torch.arange(48, device=DEV, dtype=torch.int32) % 2
+        for out in (t, t[:24], t.view(48, 512)):
+            with torch.no_grad(), scope() as state:
+                stale = second(t)
+                first(t)
+                n = out.shape[0]
+                adapter_add(out, x[:n], a, b, scaling, ids[:n], out=out)
+                got = second(t)
+                before = state.hits
+                first(t)
+                assert state.hits == before + 1
+            with torch.no_grad(), scope():
+                assert torch.equal(got, second(t.clone()))
+            assert not torch.equal(got, stale)
