@@ -482,13 +482,15 @@ py::object adapter_add(const Tensor& y, const Tensor& x, const Tensor& a, const 
 }
 
 // Strides {batch, token, head} of a [B, T, H, D] operand; those of dimensions
-// of one element are taken as 0, whatever they are.
-bool strides(const Tensor& t, int64_t* to) {
+// of one element are taken as 0, whatever they are. A layout that no kernel
+// reads, a token stride of keys or values from 2^23 on among them, is left to
+// the caller, which copies it.
+bool strides(const Tensor& t, int64_t* to, int64_t token_limit = (int64_t)1 << 23) {
   for (int i = 0; i < 3; ++i) {
     to[i] = t.size(i) > 1 ? t.stride(i) : 0;
     if (to[i] % 8) return false;
   }
-  return t.stride(3) == 1 && aligned(t);
+  return t.stride(3) == 1 && to[1] < token_limit && aligned(t);
 }
 
 py::object prefix_attention(const Tensor& q, const Tensor& pk, const Tensor& pv, const OptTensor& k, const OptTensor& v,
@@ -510,7 +512,7 @@ py::object prefix_attention(const Tensor& q, const Tensor& pk, const Tensor& pv,
   a.S = k ? k->size(1) : 0;
   const auto ok = [&](const Tensor& t) { return t.device() == dev && t.scalar_type() == type && no_grad(t); };
   if (!ok(q) || !ok(pk) || !ok(pv) || pk.size(3) != a.D || a.D % 8 || a.D < 8 || q.numel() == 0 ||
-      !strides(q, a.q_stride) || !strides(pk, a.prefix_k_stride) || !strides(pv, a.prefix_v_stride))
+      !strides(q, a.q_stride, INT64_MAX) || !strides(pk, a.prefix_k_stride) || !strides(pv, a.prefix_v_stride))
     return py::none();
   if (k) {
     if (k->dim() != 4 || v->sizes() != k->sizes() || !ok(*k) || !ok(*v) || k->size(0) != a.B || k->size(2) != a.Hkv ||

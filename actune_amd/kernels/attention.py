@@ -15,14 +15,16 @@ from .. import _block, _native
 _TYPES = (torch.bfloat16, torch.float16)
 
 
-def _operand(t):
+def _operand(t, keys):
     """t with dense heads and strides and address in whole 16 bytes, and its
     strides {batch, token, head} (0 for dimensions of one element): a copy
-    only where its layout is another, or a token's stride too long."""
+    only where its layout is another, or a token's stride of keys or values too
+    long."""
     def strides(t):
         return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
     got = strides(t)
-    if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in got) or got[1] >= 1 << 23 or t.data_ptr() % 16):
+    if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in got) or keys and got[1] >= 1 << 23
+                      or t.data_ptr() % 16):
         t = t.contiguous()
         t = t.clone() if t.data_ptr() % 16 else t
         got = strides(t)
@@ -96,7 +98,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, *, prefix_len
     held = []  # copies live until the call is made
     for name, x in operands.items():
         if x is not None:
-            x, stride = _operand(x)
+            x, stride = _operand(x, name != "q")
             held.append(x)
             setattr(args, name, _block.ptr(x))
             setattr(args, name + "_stride", stride)

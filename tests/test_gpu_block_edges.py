@@ -1,0 +1,35 @@
+"""Edges of the operators between the packed projections: layouts that are
+copied. Tolerances are those of test_gpu_block.py."""
+import pytest
+import torch
+
+import test_gpu_block as block
+from actune_amd import _block, _native
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_attention_token_strides_past_the_kernels(native, monkeypatch):
+    """Caches whose tokens lie 2^23 elements apart and more, which the kernels' offsets do not take, are copied, through
+    both bindings; one stride below is read in place."""
+    from actune_amd.kernels.attention import shared_prefix_attention
+    if not native:
+        monkeypatch.setattr(_block, "_FAST", _native._CtypesOnly())
+    gen, tokens, d = block._gen(21), 70, 64
+    q = block._normal(gen, 2, 3, 4, d, dtype=torch.bfloat16)
+    for stride in ((1 << 23) - 8, 1 << 23, (1 << 23) + 64):
+        cache = torch.empty(tokens * stride, device=DEV, dtype=torch.bfloat16)  # 1.2 GB
+        views = []
+        for at in (0, 4 * d):  # keys and values of two heads: one sequence's tokens, or every second one of two
+            rows = cache.as_strided((1, tokens, 2, d), (0, stride, d, 1), at)
+            rows.copy_(block._normal(gen, 1, tokens, 2, d, dtype=torch.bfloat16))
+            views.append(rows)
+        own = [r.as_strided((2, tokens // 2, 2, d), (tokens // 2 * stride, stride, d, 1), r.storage_offset()) for r in views]
+        dense = [r.contiguous() for r in (*views, *own)]
+        want = shared_prefix_attention(q, *dense, causal=True, return_lse=True)
+        for operands in ((*views, *own), (*views, *dense[2:]), (*dense[:2], *own)):
+            got = shared_prefix_attention(q, *operands, causal=True, return_lse=True)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), stride
