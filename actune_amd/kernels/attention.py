@@ -23,8 +23,7 @@ def _operand(t, keys):
     def strides(t):
         return [t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)]
     got = strides(t)
-    if t.numel() and (t.stride(3) != 1 or any(s % 8 for s in got) or keys and got[1] >= 1 << 23
-                      or t.data_ptr() % 16):
+    if t.stride(3) != 1 or any(s % 8 for s in got) or keys and got[1] >= 1 << 23 or t.data_ptr() % 16:
         t = t.contiguous()
         t = t.clone() if t.data_ptr() % 16 else t
         got = strides(t)
@@ -97,7 +96,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, *, prefix_len
                                 dtype=_native.DTYPE_CODES[q.dtype])
     held = []  # copies live until the call is made
     for name, x in operands.items():
-        if x is not None:
+        if x is not None and x.numel():  # (none of an empty one is read: its layout does not matter)
             x, stride = _operand(x, name != "q")
             held.append(x)
             setattr(args, name, _block.ptr(x))

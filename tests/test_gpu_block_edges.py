@@ -1,5 +1,5 @@
 """Edges of the operators between the packed projections: layouts that are
-copied. Tolerances are those of test_gpu_block.py."""
+copied or not read. Tolerances are those of test_gpu_block.py."""
 import pytest
 import torch
 
@@ -33,3 +33,19 @@ def test_attention_token_strides_past_the_kernels(native, monkeypatch):
         for operands in ((*views, *own), (*views, *dense[2:]), (*dense[:2], *own)):
             got = shared_prefix_attention(q, *operands, causal=True, return_lse=True)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), stride
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_attention_empty_operands_of_any_layout(native, monkeypatch):
+    """No own keys, or no prefix, cut from tensors whose strides no kernel reads."""
+    from actune_amd.kernels.attention import shared_prefix_attention
+    if not native:
+        monkeypatch.setattr(_block, "_FAST", _native._CtypesOnly())
+    q, pk, pv, k, v = block._attention_inputs(block._gen(22), 3, 2, 4, 2, 64, 40, 10, 1, torch.bfloat16)
+    odd = lambda t: torch.cat([t, t[..., :1]], -1)[:, 1:1, :, 1:]  # noqa: E731
+    none = odd(k)
+    assert none.shape == (3, 0, 2, 64) and none.stride(0) % 8
+    assert torch.equal(shared_prefix_attention(q, pk, pv, none, odd(v)), shared_prefix_attention(q, pk, pv))
+    assert torch.equal(shared_prefix_attention(q, odd(pk), odd(pv), k, v),
+                       shared_prefix_attention(q, pk[:, :0], pv[:, :0], k, v))
+    assert not bool(shared_prefix_attention(q, odd(pk), odd(pv), none, odd(v)).any())
