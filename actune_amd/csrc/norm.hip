@@ -21,6 +21,7 @@ namespace {
 struct NormArgs {
   actune_block_norm_args p;
   int64_t per_wg;  // rows of one workgroup (kernel of rows in registers)
+  int64_t first;   // the launch's first row (kernel of rows of any length)
 };
 
 // Row of a modulation tensor that row m reads.
@@ -172,7 +173,7 @@ __global__ __launch_bounds__(kLong) void norm_long(const NormArgs args) {
   constexpr int ES = DT == kF32 ? 4 : 2;
   __shared__ float red[2][kLong / 64];
   const actune_block_norm_args& p = args.p;
-  const int64_t D = p.D, m = blockIdx.x;
+  const int64_t D = p.D, m = args.first + blockIdx.x;
   const bool behind = p.branch && p.branch_weight;
   const void* res = byte_at(p.residual, m * p.residual_stride * ES);
   const void* br = byte_at(p.branch, m * p.branch_stride * ES);
@@ -212,6 +213,15 @@ __global__ __launch_bounds__(kLong) void norm_long(const NormArgs args) {
   }
 }
 
+// (a dispatch holds less than 2^32 threads: rows of few columns can be more)
+template <int DT>
+void launch_long(NormArgs a, hipStream_t st) {
+  for (const int64_t most = 1 << 21; a.first < a.p.M; a.first += most) {
+    const int64_t rows = a.p.M - a.first;
+    norm_long<DT><<<dim3((unsigned)(rows < most ? rows : most)), kLong, 0, st>>>(a);
+  }
+}
+
 template <int DT, int TPR, int CH>
 void launch_rows(NormArgs a, hipStream_t st) {
   constexpr int RPW = TPR > 64 ? 1 : 4;
@@ -231,16 +241,16 @@ void launch_rows(NormArgs a, hipStream_t st) {
 // 133 for 8192). Two chunks of f32 in 1024 threads do not fit the registers.
 template <int DT>
 void launch_norm(const actune_block_norm_args& p, hipStream_t st) {
-  const NormArgs a{p, 0};
+  const NormArgs a{p, 0, 0};
   const int64_t D = p.D;
-  if (D < 8) norm_long<DT><<<dim3((unsigned)p.M), kLong, 0, st>>>(a);  // (a row in registers is eights)
+  if (D < 8) launch_long<DT>(a, st);  // (a row in registers is eights)
   else if (D <= 512) launch_rows<DT, 64, 1>(a, st);
   else if (D <= 1024) launch_rows<DT, 128, 1>(a, st);
   else if (D <= 2048) launch_rows<DT, 256, 1>(a, st);
   else if (D <= 4096) launch_rows<DT, 256, 2>(a, st);
   else if (D <= 8192) launch_rows<DT, 512, 2>(a, st);
   else if (D <= 16384 && DT != kF32) launch_rows<DT, DT != kF32 ? 1024 : 512, 2>(a, st);
-  else norm_long<DT><<<dim3((unsigned)p.M), kLong, 0, st>>>(a);
+  else launch_long<DT>(a, st);
 }
 
 }  // namespace

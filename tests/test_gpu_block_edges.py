@@ -1,5 +1,5 @@
 """Edges of the operators between the packed projections: layouts that are
-copied or not read. Tolerances are those of test_gpu_block.py."""
+copied or not read, sizes past one dispatch. Tolerances are those of test_gpu_block.py."""
 import pytest
 import torch
 
@@ -49,3 +49,18 @@ def test_attention_empty_operands_of_any_layout(native, monkeypatch):
     assert torch.equal(shared_prefix_attention(q, odd(pk), odd(pv), k, v),
                        shared_prefix_attention(q, pk[:, :0], pv[:, :0], k, v))
     assert not bool(shared_prefix_attention(q, odd(pk), odd(pv), none, odd(v)).any())
+
+
+@pytest.mark.parametrize("behind", [False, True])
+def test_block_norm_rows_past_a_dispatch(behind):
+    """More rows of few columns than a dispatch has room for at one workgroup each."""
+    from actune_amd.kernels.norms import block_norm
+    dtype, rows, width = torch.bfloat16, (1 << 22) + 4099, 4
+    gen = block._gen(23)
+    x, y = block._normal(gen, rows, width, dtype=dtype), block._normal(gen, rows, width, dtype=dtype)
+    w = block._normal(gen, width, dtype=dtype)
+    bw = block._normal(gen, width, dtype=dtype) if behind else None
+    hidden, normed = block_norm(x, y, weight=w, branch_weight=bw)
+    h, n, size, nsize = block._norm64(x, y, w, bw, None, None, None, 1.0, 0.0, 1e-6)
+    block._near(hidden, h, block.UNIT[dtype] * h.abs() + 2.0 ** -18 * size, "hidden")
+    block._near(normed, n, block.UNIT[dtype] * n.abs() + 2.0 ** -18 * nsize, "normed")
