@@ -103,6 +103,7 @@ struct AttnArgs {
   actune_prefix_attention_args p;
   int parts, splits;
   int main_items;
+  int first;            // the launch's first item or, of a join, row
   int pre_cap;          // tiles of the prefix
   int per_group;        // sequences of a group
   int set_rows;         // rows of a main item's row set, and of one sequence's
@@ -1057,10 +1058,11 @@ __global__ __launch_bounds__((64 * Shape<DP, BIG>::WAVES), BIG ? 2 : 1) void att
   extern __shared__ __align__(16) uint8_t attn_lds[];
   using S = Shape<DP, BIG>;
   const actune_prefix_attention_args& p = args.p;
+  const int item = args.first + (int)blockIdx.x;
   const Keys none{nullptr, nullptr, 0, 0, nullptr, 0};
   Item it{none, none, 0, 0, 0, 0, 0, 0, 0, args.set_rows, 0, INT_MAX};
-  if (!STACKED || (int)blockIdx.x < args.main_items) {
-    int id = xcd_order((int)blockIdx.x, args.main_items);
+  if (!STACKED || item < args.main_items) {
+    int id = xcd_order(item, args.main_items);
     it.row0 = take(id, args.tiles) * S::ROWS;
     const int seq = STACKED ? 0 : take(id, args.per_group_div);
     const int split = it.part = take(id, args.splits_div);
@@ -1081,7 +1083,7 @@ __global__ __launch_bounds__((64 * Shape<DP, BIG>::WAVES), BIG ? 2 : 1) void att
       it.nb = max(0, min(c1 - args.pre_cap, (max(seen, 0) + S::KEYS - 1) / S::KEYS) - it.b0);
     }
   } else {
-    int id = (int)blockIdx.x - args.main_items;
+    int id = item - args.main_items;
     const int tile = take(id, args.own_tiles) * S::ROWS;
     const int split = take(id, args.own_splits);
     it.part = args.splits + split;
@@ -1124,7 +1126,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void join(const AttnArgs args
   constexpr int LANES = DP / 4, GROUPS = 64 / LANES * W;
   __shared__ float meet[W][6 * 64];
   const actune_prefix_attention_args& p = args.p;
-  const int64_t rows = p.B * p.T * p.Hq, row = (int64_t)blockIdx.x * (W > 1 ? 1 : 4) + (W > 1 ? 0 : threadIdx.x >> 6);
+  const int64_t rows = p.B * p.T * p.Hq, row = args.first + (int64_t)blockIdx.x * (W > 1 ? 1 : 4) + (W > 1 ? 0 : threadIdx.x >> 6);
   if (row >= rows) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = 4 * (lane % LANES), D = (int)p.D;
   const int grp = (W > 1 ? wave * (64 / LANES) : 0) + lane / LANES;
@@ -1288,12 +1290,29 @@ int64_t need_bytes(const actune_prefix_attention_args& p, const Plan& g) {
   return g.parts == 1 ? 0 : ml_bytes(p, g) + g.parts * part_rows(p) * padded(p.D) * 4;
 }
 
+// Items or rows of a launch: a dispatch holds less than 2^32 threads.
+constexpr int64_t kMost = 1 << 21;
+
 template <int DT, int DP, bool BIG, bool STACKED>
-void launch_attend(const AttnArgs& a, int64_t grid, hipStream_t st) {
+void launch_attend(AttnArgs a, int64_t items, hipStream_t st) {
   using S = Shape<DP, BIG>;
   if constexpr (S::LDS > 64 * 1024) allow_dynamic_lds<attend<DT, DP, BIG, STACKED>>(160 * 1024);
   constexpr int threads = 64 * S::WAVES, lds = S::LDS;
-  attend<DT, DP, BIG, STACKED><<<dim3((unsigned)grid), threads, lds, st>>>(a);
+  for (int64_t first = 0; first < items; first += kMost) {
+    a.first = (int)first;
+    const int64_t n = items - first < kMost ? items - first : kMost;
+    attend<DT, DP, BIG, STACKED><<<dim3((unsigned)n), threads, lds, st>>>(a);
+  }
+}
+
+template <int DT, int DP, int W>
+void launch_join(AttnArgs a, int64_t rows, hipStream_t st) {
+  constexpr int each = W > 1 ? 1 : 4;  // rows of a workgroup
+  for (int64_t first = 0; first < rows; first += kMost * each) {
+    a.first = (int)first;
+    const int64_t left = (rows - first + each - 1) / each, n = left < kMost ? left : kMost;
+    join<DT, DP, W><<<dim3((unsigned)n), W > 4 ? 64 * W : 256, 0, st>>>(a);
+  }
 }
 
 template <int DT, int DP>
@@ -1308,9 +1327,9 @@ void launch(const AttnArgs& a, const Plan& g, hipStream_t st) {
   }
   const int64_t rows = part_rows(a.p);
   constexpr int ROUND = 4 * 64 / (DP / 4);  // parts that a wave has in flight
-  if (g.parts > 8 * ROUND) join<DT, DP, 16><<<dim3((unsigned)rows), 1024, 0, st>>>(a);
-  else if (g.parts > ROUND) join<DT, DP, 4><<<dim3((unsigned)rows), 256, 0, st>>>(a);
-  else if (g.parts > 1) join<DT, DP, 1><<<dim3((unsigned)((rows + 3) / 4)), 256, 0, st>>>(a);
+  if (g.parts > 8 * ROUND) launch_join<DT, DP, 16>(a, rows, st);
+  else if (g.parts > ROUND) launch_join<DT, DP, 4>(a, rows, st);
+  else if (g.parts > 1) launch_join<DT, DP, 1>(a, rows, st);
 }
 
 template <int DT>

@@ -64,3 +64,23 @@ def test_block_norm_rows_past_a_dispatch(behind):
     h, n, size, nsize = block._norm64(x, y, w, bw, None, None, None, 1.0, 0.0, 1e-6)
     block._near(hidden, h, block.UNIT[dtype] * h.abs() + 2.0 ** -18 * size, "hidden")
     block._near(normed, n, block.UNIT[dtype] * n.abs() + 2.0 ** -18 * nsize, "normed")
+
+
+@pytest.mark.parametrize("b,heads,p,s,g", [((1 << 18) + 1, 16, 5, 2, 1), ((1 << 20) + 1, 16, 12, 2, 1),
+                                           ((1 << 21) + 5, 1, 3, 1, (1 << 21) + 5)])
+def test_attention_batches_past_a_dispatch(b, heads, p, s, g):
+    """More items, and more rows to join, than one dispatch takes."""
+    from actune_amd.kernels.attention import shared_prefix_attention
+    gen, d, dtype = block._gen(24), 8, torch.bfloat16
+    q, pk, pv, k, v = block._attention_inputs(gen, b, 1, heads, heads, d, p, s, g, dtype)
+    got, lse = shared_prefix_attention(q, pk, pv, k, v, return_lse=True)
+    per = b // g
+    for first in range(0, b, 1 << 17):
+        rows = slice(first, min(b, first + (1 << 17)))
+        keys, vals = (torch.cat([(x[rows] if per == 1 else x.expand(b, -1, -1, -1)[rows]), y[rows]], 1).double()
+                      for x, y in ((pk, k), (pv, v)))
+        scores = (q[rows].double() * keys).sum(-1) * d ** -0.5  # (one query: [B, keys, heads])
+        pr = torch.softmax(scores, 1)[..., None]
+        want, size = (pr * vals).sum(1), (pr * vals.abs()).sum(1)
+        block._near(got[rows, 0], want, block.UNIT[dtype] * want.abs() + (block.UNIT[dtype] + 1e-4) * size, first)
+        block._near(lse[rows, 0], torch.logsumexp(scores, 1), 1e-4, first)
