@@ -509,7 +509,8 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int64_t R) {
   Plan g;
   g.RP = (int)((R + 15) / 16) * 16;
   const int64_t rounds = (M * ((N + kOneColumns - 1) / kOneColumns) + kCus - 1) / kCus;
-  g.one = M <= 64 && R <= kOneRank && rounds * g.RP * K <= 65536;
+  // (a grid's y stays below 2^16)
+  g.one = M <= 64 && R <= kOneRank && rounds * g.RP * K <= 65536 && N <= kOneColumns * 65535;
   const int64_t steps = (K + 255) / 256, blocks = (N + 255) / 256;
   auto groups = [&](int64_t t) { return (M + t - 1) / t; };
   g.down_tokens = M <= 64 ? 1 : groups(16 * kDownTiles) * (steps < 16 ? steps : 16) < 2 * kCus ? 16 : 16 * kDownTiles;
@@ -538,8 +539,10 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int64_t R) {
   return g;
 }
 
+// (a dispatch holds less than 2^32 threads: 2^24 workgroups of up_tiles(R) 16s of tokens)
 bool sizes_ok(int64_t M, int64_t N, int64_t K, int64_t R) {
-  return M >= 0 && M <= INT_MAX / 2 && N > 0 && N <= INT_MAX / 2 && K > 0 && K <= INT_MAX / 2 && R > 0 && R <= kMaxRank;
+  return M >= 0 && N > 0 && N <= INT_MAX / 2 && K > 0 && K <= INT_MAX / 2 && R > 0 && R <= kMaxRank &&
+         M <= (int64_t)16 * up_tiles(R) * ((1 << 24) - 1);
 }
 
 template <int DT, int NT>
