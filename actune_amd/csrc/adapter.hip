@@ -602,6 +602,8 @@ int actune_adapter_add(const actune_adapter_args* args, void* stream) {
     if (s < 0 || s > most) return block_fail("invalid row stride");
   if (p.ids_rows < 1 || p.ids_rows > INT_MAX) return block_fail("an id covers one row at least");
   if (p.out_stride < p.N && p.M > 1) return block_fail("rows of out overlap");
+  // (its rows would be written where others of y are yet to be read)
+  if (p.out && p.out == p.y && p.out_stride != p.y_stride && p.M > 1) return block_fail("out on y needs y's row stride");
   if (p.M == 0) return kOk;
   if (!p.x || !p.y || !p.ids || !p.out || (p.L > 0 && (!p.a || !p.b || !p.scaling))) return block_fail("null pointer");
   const Plan g = plan_of(p.M, p.N, p.K, p.R);

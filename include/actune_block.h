@@ -74,10 +74,10 @@ int actune_block_norm(const actune_block_norm_args* args, void* stream);
  * in the second product; out is rounded once. An adapter's values reach only
  * the rows that name it, whatever they are.
  *
- * x: [M, K] and y, out: [M, N] with row strides (out may be y itself); a:
- * [L, R, K], b: [L, N, R], both dense; scaling: f32 [L]; ids: int32, one for
- * each ids_rows rows. x, y, a, b and out have one dtype, bf16 or f16.
- * 1 <= R <= 128.
+ * x: [M, K] and y, out: [M, N] with row strides (out may be y itself, with
+ * y's row stride); a: [L, R, K], b: [L, N, R], both dense; scaling: f32 [L];
+ * ids: int32, one for each ids_rows rows. x, y, a, b and out have one dtype,
+ * bf16 or f16. 1 <= R <= 128.
  * workspace: actune_adapter_workspace_bytes(M, N, K, R) bytes, 16-byte
  * aligned, no other call's at the same time.
  */

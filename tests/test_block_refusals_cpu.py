@@ -15,3 +15,12 @@ def test_adapter_tokens_end_where_a_dispatch_ends(rank, most):
                               ids_rows=1, M=most + 1, N=64, K=64, R=rank, L=2, dtype=0)
     assert _block.lib().actune_adapter_add(args, None) == 1
     assert "dimensions" in _block.lib().actune_block_last_error().decode()
+
+
+@pytest.mark.parametrize("tokens,out_stride,message", [(4, 64, "y's row stride"), (4, 80, "workspace"), (1, 64, "workspace")])
+def test_adapter_out_on_y_takes_the_stride_of_y(tokens, out_stride, message):
+    """Rows written over others of y would be read as y, and rows without an adapter would not be moved."""
+    args = _block.AdapterArgs(x=16, y=1024, a=16, b=16, scaling=16, ids=16, out=1024, x_stride=64, y_stride=80,
+                              out_stride=out_stride, ids_rows=1, M=tokens, N=64, K=64, R=8, L=2, dtype=0)
+    assert _block.lib().actune_adapter_add(args, None) == 1
+    assert message in _block.lib().actune_block_last_error().decode()
