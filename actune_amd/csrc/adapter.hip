@@ -198,7 +198,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args
   const actune_adapter_args& p = args.p;
   constexpr int TOK = 16 * NT, CH = 4 * KS;  // tokens; 8-element chunks of a row of low
   __shared__ u16x8 low[NT][KS][2][64];       // operand fragments of hi and lo
-  __shared__ float by[TOK];
+  __shared__ float2 by[TOK];                 // a token's scaling, and the power of two that its low is short of
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, q = lane >> 4;
   const int2 wg = item();
@@ -247,7 +247,7 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args
     low[c / 16][s][1][at] = lo;
     if (ch == 0) {
       const int own = there ? p.ids[(uint32_t)(m0 + c) / (uint32_t)p.ids_rows] : -1;
-      by[c] = own >= 0 && own < L ? p.scaling[own] * __uint_as_float((uint32_t)(127 + e2) << 23) : 0.f;
+      by[c] = make_float2(own >= 0 && own < L ? p.scaling[own] : 0.f, __uint_as_float((uint32_t)(127 + e2) << 23));
     }
   }
   __syncthreads();
@@ -307,12 +307,12 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args
         }
         if ((same >> (16 * t + col)) & 1) {
           uint16_t* to = (uint16_t*)p.out + (m0 + 16 * t + col) * p.out_stride;
-          const float w = by[16 * t + col];
+          const float2 w = by[16 * t + col];
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = fmaf(w, acc[2 * k + (i >> 2)][i & 3], raw_at<DT>(y[t][k], i));
+            for (int i = 0; i < 8; ++i) f[i] = fmaf(w.x, w.y * acc[2 * k + (i >> 2)][i & 3], raw_at<DT>(y[t][k], i));
             if (at + 32 * k < N) store_raw<DT>(to, at + 32 * k, N, f);
           }
         }

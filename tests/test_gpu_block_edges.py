@@ -1,5 +1,5 @@
 """Edges of the operators between the packed projections: layouts that are
-copied or not read, sizes past one dispatch. Tolerances are those of test_gpu_block.py."""
+copied or not read, sizes past one dispatch, values at the ends of their range. Tolerances are those of test_gpu_block.py."""
 import pytest
 import torch
 
@@ -84,3 +84,25 @@ def test_attention_batches_past_a_dispatch(b, heads, p, s, g):
         want, size = (pr * vals).sum(1), (pr * vals.abs()).sum(1)
         block._near(got[rows, 0], want, block.UNIT[dtype] * want.abs() + (block.UNIT[dtype] + 1e-4) * size, first)
         block._near(lse[rows, 0], torch.logsumexp(scores, 1), 1e-4, first)
+
+
+# one launch; two: a token a workgroup, tiles of 16, of 64 and (rank above 64) of 32 tokens
+ADAPTER_FORMS = [(5, 512, 96, 16), (5, 512, 96, 40), (5, 512, 96, 100), (70, 512, 96, 16), (70, 520, 100, 128),
+                 (2100, 8200, 2100, 16), (2100, 8200, 2100, 64), (2100, 8200, 1030, 128)]
+
+
+@pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
+def test_adapter_factors_far_apart(m, k, n, r):
+    """A large low-rank product, a small B and a scaling whose product with the first passes f32's range, and the other
+    way round: the result is in range and stays so."""
+    from actune_amd.kernels.adapters import adapter_add
+    gen, dtype = block._gen(27), torch.bfloat16
+    y = torch.zeros(m, n, device=DEV, dtype=dtype)
+    ids = torch.zeros(m, device=DEV, dtype=torch.int32)
+    for low, up, scale in ((2.0 ** 54, 2.0 ** -90, 2.0 ** 20), (2.0 ** -50, 2.0 ** 110, 2.0 ** -24), (2.0 ** -45, 2.0 ** 90, 2.0 ** -40)):
+        x, a = block._normal(gen, m, k, dtype=dtype, by=low), block._normal(gen, 1, r, k, dtype=dtype, by=low)
+        b = block._normal(gen, 1, n, r, dtype=dtype, by=up)
+        scaling = torch.full((1,), scale, device=DEV)
+        want, tol = block._adapter64(y, x, a, b, scaling, ids)
+        assert bool(want.abs().max() < 3e38) and bool(want.abs().max() > 1e-30)
+        block._near(adapter_add(y, x, a, b, scaling, ids), want, tol + block.UNIT[dtype] * want.abs())
