@@ -83,6 +83,12 @@ __device__ __forceinline__ int token_id(const actune_adapter_args& p, int tokens
   const int64_t m = m0 + lane;  // (below 2^31)
   return lane < tokens && m < p.M ? p.ids[(uint32_t)m / (uint32_t)p.ids_rows] : -1;
 }
+// two values to the 16-bit type, toward zero, a in the low half
+template <int DT>
+__device__ __forceinline__ uint32_t toward_zero(float a, float b) {
+  if constexpr (DT == kBF16) return (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u);
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
 __device__ __forceinline__ u16x8 load8(const uint16_t* p) { return *(const u16x8_any*)p; }
 
 // down: one split of K, the four waves a quarter each in steps of 64 (two MFMAs
@@ -189,16 +195,21 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_down(const AdapterArgs ar
 // up: a wave takes 64 columns at a time: four products t whose rows stand for
 // columns 32 (t / 2) + 8 (row / 4) + 4 (t % 2) + row % 4, so that a lane ends
 // with two runs of 8 columns of its token, and the four lanes of a token with 64
-// consecutive bytes of each half. low is held as hi + lo of the 16-bit type under a power
-// of two that brings its row's largest value to [1, 2): no range is lost, and
-// the second product's error stays near f32's (2^-17 of a value in bf16, 2^-22
-// of the largest in f16).
+// consecutive bytes of each half. low is held as hi + lo of the 16-bit type under
+// a power of two that brings its row's largest finite value to the type's middle
+// (f16: below its end by the factor that keeps small values out of its
+// subnormals; bf16: where 128 products of its largest values stay finite): no
+// range is lost, and the second product's error stays near f32's (2^-16 of a
+// value in bf16, 2^-21 in f16). hi is rounded toward zero, lo has its sign, and
+// neither is zero where low is not: an infinity of B then gives both products
+// the formula's sign, where a zero or another sign would make their sum NaN.
 template <int DT, int KS, int NT>
 __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args) {
   const actune_adapter_args& p = args.p;
   constexpr int TOK = 16 * NT, CH = 4 * KS;  // tokens; 8-element chunks of a row of low
   __shared__ u16x8 low[NT][KS][2][64];       // operand fragments of hi and lo
   __shared__ float2 by[TOK];                 // a token's scaling, and the power of two that its low is short of
+  constexpr int kTop = DT == kF16 ? 14 : -9;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int col = lane & 15, q = lane >> 4;
   const int2 wg = item();
@@ -226,28 +237,35 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args
     }
     float top = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]));
+    for (int j = 0; j < 8; ++j) top = fmaxf(top, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
 #pragma unroll
     for (int d = 1; d < CH; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
-    // 2^-e with top in [2^e, 2^(e + 1)); zeros, infinities and NaN go as they are
+    // the largest finite value to [2^kTop, 2^(kTop + 1))
     int e2 = (int)((__float_as_uint(top) >> 23) & 0xffu) - 127;
-    if (e2 == -127 || e2 == 128) e2 = 0;
-    e2 = min(max(e2, -120), 120);
-    const float down = __uint_as_float((uint32_t)(127 - e2) << 23);
-    u16x8 hi, lo;
+    e2 = top == 0.f ? 0 : min(max(e2, -112), 117);
+    const float down = __uint_as_float((uint32_t)(127 + kTop - e2) << 23);
+    u16x8 hi, lo, some;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float v = f[j] * down;
-      hi[j] = to16<DT>(v);
-      const float rest = v - raw_at<DT>(Raw8<DT>{hi}, j);
-      lo[j] = to16<DT>(rest == rest ? rest : 0.f);  // (infinity - infinity)
+    for (int j = 0; j < 8; j += 2) {
+      const float v[2] = {f[j] * down, f[j + 1] * down};
+      const uint32_t both = toward_zero<DT>(v[0], v[1]);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        hi[j + k] = (uint16_t)(both >> (16 * k));
+        const float rest = v[k] - raw_at<DT>(Raw8<DT>{hi}, j + k);
+        lo[j + k] = to16<DT>(rest == rest ? rest : 0.f);  // (infinity - infinity)
+        some[j + k] = (uint16_t)min(__float_as_uint(f[j + k]) << 1, 1u);  // (0 for zeros)
+      }
     }
+    const u16x8 sign = hi & 0x8000;
+    hi = sign | __builtin_elementwise_max((u16x8)(hi & 0x7fff), some);
+    lo = sign | __builtin_elementwise_max((u16x8)(lo & 0x7fff), some);
     const int at = 16 * (ch % 4) + c % 16;
     low[c / 16][s][0][at] = hi;
     low[c / 16][s][1][at] = lo;
     if (ch == 0) {
       const int own = there ? p.ids[(uint32_t)(m0 + c) / (uint32_t)p.ids_rows] : -1;
-      by[c] = make_float2(own >= 0 && own < L ? p.scaling[own] : 0.f, __uint_as_float((uint32_t)(127 + e2) << 23));
+      by[c] = make_float2(own >= 0 && own < L ? p.scaling[own] : 0.f, __uint_as_float((uint32_t)(127 - kTop + e2) << 23));
     }
   }
   __syncthreads();

@@ -68,11 +68,12 @@ int actune_block_norm(const actune_block_norm_args* args, void* stream);
 
 /*
  * out[m] = y[m] + scaling[id] * B[id] (A[id] x[m]) with id =
- * ids[m / ids_rows]; a row whose id is not in [0, L) gets out[m] = y[m]. Products of the 16-bit
- * inputs are exact and summed in f32; A x is held as two 16-bit parts (about
- * 16 bits of mantissa in bf16, 22 in f16) under one power of two for each row
- * in the second product; out is rounded once. An adapter's values reach only
- * the rows that name it, whatever they are.
+ * ids[m / ids_rows]; a row whose id is not in [0, L) gets
+ * out[m] = y[m]. Products of the 16-bit inputs are exact and summed in f32;
+ * A x is held as two 16-bit parts (about 16 bits of mantissa in bf16, 21 in
+ * f16) under one power of two for each row in the second product; out is
+ * rounded once. Infinities and NaN give what the formula gives. An adapter's
+ * values reach only the rows that name it, whatever they are.
  *
  * x: [M, K] and y, out: [M, N] with row strides (out may be y itself, with
  * y's row stride); a: [L, R, K], b: [L, N, R], both dense; scaling: f32 [L];

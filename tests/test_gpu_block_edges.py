@@ -91,6 +91,38 @@ ADAPTER_FORMS = [(5, 512, 96, 16), (5, 512, 96, 40), (5, 512, 96, 100), (70, 512
                  (2100, 8200, 2100, 16), (2100, 8200, 2100, 64), (2100, 8200, 1030, 128)]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
+def test_adapter_infinities_and_nan_are_the_formulas(m, k, n, r, dtype):
+    """Infinities and NaN in B, in A and in x, beside low-rank products beyond f16's range and of zero: each output is
+    infinite, NaN or finite as the formula's is, and the rows of other adapters keep their bits."""
+    from actune_amd.kernels.adapters import adapter_add
+    gen, inf, nan = block._gen(26), float("inf"), float("nan")
+    x, y = block._normal(gen, m, k, dtype=dtype, by=16.0), block._normal(gen, m, n, dtype=dtype)
+    a, b = block._normal(gen, 3, r, k, dtype=dtype, by=32.0), block._normal(gen, 3, n, r, dtype=dtype)
+    x[:, :8] = (x[:, :8].abs() + 1).to(dtype)
+    a[:, 3] = 0                       # (a low-rank product of zero: 0 times an infinity is NaN)
+    scaling = torch.tensor([1e-3, -1e-3, 1e-3], device=DEV)
+    ids = torch.arange(m, device=DEV, dtype=torch.int32) % 4 - 1
+    clean = adapter_add(y, x, a, b, scaling, ids)
+    b[0, 5, 1], b[0, 17, 2], b[0, 30, 4], b[0, 40, 3] = inf, -inf, nan, inf
+    b[0, 50, 1], b[0, 50, 2] = inf, -inf
+    a[1, 2, 7] = inf                  # (x[:, 7] is at least 1: this product is infinite in every row of adapter 1)
+    want, tol = block._adapter64(y, x, a, b, scaling, ids)
+    got = adapter_add(y, x, a, b, scaling, ids)
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(want)), kind
+    other = (ids != 0) & (ids != 1)
+    assert torch.equal(got[other], clean[other])
+    columns = [i for i in range(n) if i not in (5, 17, 30, 40, 50)]
+    rows = ids == 0
+    assert torch.equal(got[rows][:, columns], clean[rows][:, columns])
+    x[2, 9] = inf                     # (ids[2] is 1; one row alone)
+    again = adapter_add(y, x, a, b, scaling, ids)
+    kept = torch.arange(m, device=DEV) != 2
+    assert torch.equal(again[kept].nan_to_num(), got[kept].nan_to_num())
+
+
 @pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
 def test_adapter_factors_far_apart(m, k, n, r):
     """A large low-rank product, a small B and a scaling whose product with the first passes f32's range, and the other
