@@ -92,6 +92,22 @@ ADAPTER_FORMS = [(5, 512, 96, 16), (5, 512, 96, 40), (5, 512, 96, 100), (70, 512
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("by", [2.0 ** -20, 1.0, 2.0 ** 9])
+@pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
+def test_adapter_low_products_keep_their_range_in_every_form(m, k, n, r, by, dtype):
+    """Low-rank products far above and below f16's range, in each way to form them. The bound is that of
+    test_gpu_block.py: 2^-15 of the largest |a| |x| times |b|, and the output's rounding."""
+    from actune_amd.kernels.adapters import adapter_add
+    gen = block._gen(25)
+    x, y = block._normal(gen, m, k, dtype=dtype, by=min(by, 1.0) * 8), torch.zeros(m, n, device=DEV, dtype=dtype)
+    a, b = block._normal(gen, 2, r, k, dtype=dtype, by=max(by, 1.0)), block._normal(gen, 2, n, r, dtype=dtype)
+    scaling = torch.full((2,), 1.0 / (k * by), device=DEV)
+    ids = torch.arange(m, device=DEV, dtype=torch.int32) // 3 % 2
+    want, tol = block._adapter64(y, x, a, b, scaling, ids)
+    block._near(adapter_add(y, x, a, b, scaling, ids), want, tol + block.UNIT[dtype] * want.abs() + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
 def test_adapter_infinities_and_nan_are_the_formulas(m, k, n, r, dtype):
     """Infinities and NaN in B, in A and in x, beside low-rank products beyond f16's range and of zero: each output is
@@ -138,3 +154,20 @@ def test_adapter_factors_far_apart(m, k, n, r):
         want, tol = block._adapter64(y, x, a, b, scaling, ids)
         assert bool(want.abs().max() < 3e38) and bool(want.abs().max() > 1e-30)
         block._near(adapter_add(y, x, a, b, scaling, ids), want, tol + block.UNIT[dtype] * want.abs())
+
+
+@pytest.mark.parametrize("m,k,n,r", ADAPTER_FORMS)
+def test_adapters_keep_to_their_rows_in_every_form(m, k, n, r):
+    """A broken adapter, a broken scaling and a broken row reach the rows that name them and no others."""
+    from actune_amd.kernels.adapters import adapter_add
+    gen, dtype = block._gen(28), torch.float16
+    x, y = block._normal(gen, m, k, dtype=dtype), block._normal(gen, m, n, dtype=dtype)
+    a, b = block._normal(gen, 3, r, k, dtype=dtype), block._normal(gen, 3, n, r, dtype=dtype)
+    scaling = torch.full((3,), 1.0 / k, device=DEV)
+    ids = torch.arange(m, device=DEV, dtype=torch.int32) % 4 - 1
+    want = adapter_add(y, x, a, b, scaling, ids)
+    a[1, 3, 5], b[1, 7, 2], x[1, 9], scaling[1] = torch.inf, torch.nan, torch.nan, torch.inf
+    got = adapter_add(y, x, a, b, scaling, ids)
+    kept = (ids != 1) & (torch.arange(m, device=DEV) != 1)
+    assert torch.equal(got[kept], want[kept])
+    assert bool(got[ids == 1].isnan().any()) and bool(got[1].isnan().all())
