@@ -178,6 +178,8 @@ struct Keys {
   int end;                    // keys that exist
 };
 
+__device__ const v4u kZeros = {0, 0, 0, 0};
+
 // DMA loads of tiles of KT rows, BLOCKS KiB of each by a wave: block i holds
 // rows (wave BLOCKS + i) 512 / DP on. Rows past the end read the last row that
 // exists (their scores are masked and their values cleared).
@@ -208,14 +210,34 @@ struct Loader {
     const int row0 = min(first, end - 1);  // in range also where the whole tile lies past the end
     return Tile{(const uint8_t*)src + (uint64_t)(uint32_t)row0 * stride, stride, end - 1 - row0, at};
   }
-  __device__ __forceinline__ void request(const Tile& t, int i) const {
-    uint32_t c = chunk ^ (16 * swizzle<DP>(i * RPB));
-    c = c < width ? c : 0;  // columns past D: any data of the row, met by zeros of q or not stored
-    dma16(t.base, __umul24((uint32_t)min(row + i * RPB, t.last), t.stride) + c, lds + t.at + i * 1024);
-  }
-  __device__ __forceinline__ void request(const Tile& t) const {
+  __device__ __forceinline__ uint32_t column(int i) const { return chunk ^ (16 * swizzle<DP>(i * RPB)); }
+  // Keys: columns past D are zeros, as those of q are (an infinity there would make the score NaN). A wave with few
+  // blocks leaves out the lanes that stand for them, whose places clear_columns has written; one that loads a whole
+  // tile reads zeros instead, since clearing 32 blocks takes 1 us of a short call (8 prompts of 512, 12 heads of 80,
+  // 2050 keys: 85 us without the lanes, 89.5 with zeros; a chunk of 50, 8 heads of 200, 816 keys: 16.1 and 15.1).
+  static constexpr bool ZEROS = WAVES == 1;
+  __device__ __forceinline__ void request_keys(const Tile& t) const {
 #pragma unroll
-    for (int i = 0; i < BLOCKS; ++i) request(t, i);
+    for (int i = 0; i < BLOCKS; ++i) {
+      const uint32_t c = column(i), from = __umul24((uint32_t)min(row + i * RPB, t.last), t.stride) + c;
+      if (ZEROS && width < 2 * DP) dma16(c < width ? t.base + from : (const uint8_t*)&kZeros, lds + t.at + i * 1024);
+      else if (c < width) dma16(t.base, from, lds + t.at + i * 1024);
+    }
+  }
+  // zeros past D in this wave's blocks of the place at `to`
+  __device__ __forceinline__ void clear_columns(uint8_t* to) const {
+    if (ZEROS || width == 2 * DP) return;
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i)
+      if (column(i) >= width) *(u16x8*)(to + i * 1024 + 16 * (threadIdx.x & 63)) = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+  }
+  // Values: past D any data of the row, in columns that are not stored.
+  __device__ __forceinline__ void request_values(const Tile& t) const {
+#pragma unroll
+    for (int i = 0; i < BLOCKS; ++i) {
+      const uint32_t c = column(i);
+      dma16(t.base, __umul24((uint32_t)min(row + i * RPB, t.last), t.stride) + (c < width ? c : 0), lds + t.at + i * 1024);
+    }
   }
 };
 
@@ -614,14 +636,14 @@ struct Small {
   static constexpr int TILE = 32 * DP * 2, STAGE = 2 * TILE, LDS = 2 * STAGE * WK;
 };
 
-template <int DT, int DP, int WK, bool STACKED>
+template <int DT, int DP, int WK, bool STACKED, bool FULL>
 __device__ __forceinline__ void sweep_small(const AttnArgs& args, uint8_t* lds, const Item& it) {
   using G = Small<DP, WK>;
   constexpr int OB = DP / 32;
   const actune_prefix_attention_args& p = args.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int q = lane & 31, h = lane >> 5;
-  const int D = (int)p.D;
+  const int D = FULL ? DP : (int)p.D;
   const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 2 * G::STAGE;
   uint8_t* const mem = lds + wave * 2 * G::STAGE;
   const Loader<DP, 32, 1> loader(D, 0, base);
@@ -635,8 +657,8 @@ __device__ __forceinline__ void sweep_small(const AttnArgs& args, uint8_t* lds, 
     const int first = first_of(j), key = first + lane;
     there = lane < 32 && key < s.end;
     if (there && s.mask) there = s.mask[key];  // (used a tile later: nothing waits here)
-    loader.request(L::tile(s.k, s.k_bytes, first, s.end, (j & 1) * G::STAGE));
-    loader.request(L::tile(s.v, s.v_bytes, first, s.end, (j & 1) * G::STAGE + G::TILE));
+    loader.request_keys(L::tile(s.k, s.k_bytes, first, s.end, (j & 1) * G::STAGE));
+    loader.request_values(L::tile(s.v, s.v_bytes, first, s.end, (j & 1) * G::STAGE + G::TILE));
   };
   if (n > 0) request(0);
   const Row row = row_of<STACKED>(args, it.group_or_seq, it.head, it.row0 + q, it.end);
@@ -779,7 +801,7 @@ struct Big {
   static_assert(WAVES * 8192 <= PLAIN, "the rows' way out fits");
 };
 
-template <int DT, int DP, bool STACKED>
+template <int DT, int DP, bool STACKED, bool FULL>
 __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, const Item& it) {
   using G = Big<DP>;
   using L = Loader<DP, G::KT, G::WAVES>;
@@ -790,7 +812,7 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
   const actune_prefix_attention_args& p = args.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rg = PAIR ? wave >> 1 : wave, hf = PAIR ? wave & 1 : 0, q = lane & 31, h = lane >> 5;
-  const int D = (int)p.D;
+  const int D = FULL ? DP : (int)p.D;
   const L loader(D, wave, (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds);
   const int n = it.na + it.nb;
   auto first_of = [&](int j) { return (j < it.na ? it.a0 + j : it.b0 + j - it.na) * KT; };
@@ -812,9 +834,11 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
   };
   uint64_t bits = 0, next_bits = 0;
   if (n > 0) {
-    loader.request(key_tile(0));
-    if (PAIR && n > 1) loader.request(key_tile(1));
+    loader.request_keys(key_tile(0));
+    if (PAIR && n > 1) loader.request_keys(key_tile(1));
   }
+  loader.clear_columns(lds + wave * L::BLOCKS * 1024);
+  loader.clear_columns(lds + G::TILE + wave * L::BLOCKS * 1024);
   const Row row = row_of<STACKED>(args, it.group_or_seq, it.head, it.row0 + 32 * rg + q, it.end);
   const bool busy = __any(row.live);  // (the same for both waves of a pair; the others only load)
   // queries by whole rows: a wave's (PAIR: its half of the pair's) rows to LDS
@@ -867,7 +891,7 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
     if (D < DP && 16 * s + 8 * h >= D) qf[s] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
   }
   barrier();
-  if (n > 0) loader.request(value_tile(0));
+  if (n > 0) loader.request_values(value_tile(0));
   // scores of a tile without what stands beside them, masked, and their maximum
   auto score = [&](int j) {
 #pragma unroll
@@ -932,7 +956,7 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
     if (h == 0) maxima[wave * 32 + q] = top;
     barrier();
     top = fmaxf(top, maxima[(wave ^ 1) * 32 + q]);
-    if (n > 2) loader.request(key_tile(2));
+    if (n > 2) loader.request_keys(key_tile(2));
     barrier();
     for (int j = 0; j + 1 < n; ++j) {
       const uint8_t* const kt = lds + ((j + 1) & 1) * G::TILE;
@@ -958,8 +982,8 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
       barrier();
       clear_masked(vt, j);
       const uint64_t ahead = __ballot(there != 0);
-      loader.request(value_tile(j + 1));
-      if (j + 3 < n) loader.request(key_tile(j + 3));
+      loader.request_values(value_tile(j + 1));
+      if (j + 3 < n) loader.request_keys(key_tile(j + 3));
       if (busy) sum_values(vt, pf);
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (lane == 0) turns[wave] = j + 1;
@@ -987,8 +1011,8 @@ __device__ __forceinline__ void sweep_big(const AttnArgs& args, uint8_t* lds, co
       const uint64_t ahead = __ballot(there != 0);
       if (j + 1 < n) {
         if (j + 2 < n) there = flag(j + 2);
-        loader.request(key_tile(j + 1));
-        loader.request(value_tile(j + 1));
+        loader.request_keys(key_tile(j + 1));
+        loader.request_values(value_tile(j + 1));
       }
       uint8_t* const vt = lds + (2 + (j & 1)) * G::TILE;
       clear_masked(vt, j);
@@ -1053,7 +1077,7 @@ struct Shape {
 
 // Items in order: main items by group, key head, key split, (joint: sequence),
 // row tile; then, stacked, the own keys' by sequence, head, split, row tile.
-template <int DT, int DP, bool BIG, bool STACKED>
+template <int DT, int DP, bool BIG, bool STACKED, bool FULL>
 __global__ __launch_bounds__((64 * Shape<DP, BIG>::WAVES), BIG ? 2 : 1) void attend(const AttnArgs args) {
   extern __shared__ __align__(16) uint8_t attn_lds[];
   using S = Shape<DP, BIG>;
@@ -1097,8 +1121,8 @@ __global__ __launch_bounds__((64 * Shape<DP, BIG>::WAVES), BIG ? 2 : 1) void att
     it.b0 = start_of(args.own_cut, split);
     it.nb = max(0, min(start_of(args.own_cut, split + 1), (it.own.end + S::KEYS - 1) / S::KEYS) - it.b0);
   }
-  if constexpr (BIG) sweep_big<DT, DP, STACKED>(args, attn_lds, it);
-  else sweep_small<DT, DP, S::WAVES, STACKED>(args, attn_lds, it);
+  if constexpr (BIG) sweep_big<DT, DP, STACKED, FULL>(args, attn_lds, it);
+  else sweep_small<DT, DP, S::WAVES, STACKED, FULL>(args, attn_lds, it);
 }
 
 // Joins the parts of a row in one pass: DP / 4 lanes hold four columns each,
@@ -1293,15 +1317,15 @@ int64_t need_bytes(const actune_prefix_attention_args& p, const Plan& g) {
 // Items or rows of a launch: a dispatch holds less than 2^32 threads.
 constexpr int64_t kMost = 1 << 21;
 
-template <int DT, int DP, bool BIG, bool STACKED>
+template <int DT, int DP, bool BIG, bool STACKED, bool FULL>
 void launch_attend(AttnArgs a, int64_t items, hipStream_t st) {
   using S = Shape<DP, BIG>;
-  if constexpr (S::LDS > 64 * 1024) allow_dynamic_lds<attend<DT, DP, BIG, STACKED>>(160 * 1024);
+  if constexpr (S::LDS > 64 * 1024) allow_dynamic_lds<attend<DT, DP, BIG, STACKED, FULL>>(160 * 1024);
   constexpr int threads = 64 * S::WAVES, lds = S::LDS;
   for (int64_t first = 0; first < items; first += kMost) {
     a.first = (int)first;
     const int64_t n = items - first < kMost ? items - first : kMost;
-    attend<DT, DP, BIG, STACKED><<<dim3((unsigned)n), threads, lds, st>>>(a);
+    attend<DT, DP, BIG, STACKED, FULL><<<dim3((unsigned)n), threads, lds, st>>>(a);
   }
 }
 
@@ -1315,16 +1339,24 @@ void launch_join(AttnArgs a, int64_t rows, hipStream_t st) {
   }
 }
 
-template <int DT, int DP>
-void launch(const AttnArgs& a, const Plan& g, hipStream_t st) {
+template <int DT, int DP, bool FULL>
+void launch_sweep(const AttnArgs& a, const Plan& g, hipStream_t st) {
   const int64_t grid = g.main_items + g.own_items;
   if (g.big) {
-    if (g.stacked) launch_attend<DT, DP, true, true>(a, grid, st);
-    else launch_attend<DT, DP, true, false>(a, grid, st);
+    if (g.stacked) launch_attend<DT, DP, true, true, FULL>(a, grid, st);
+    else launch_attend<DT, DP, true, false, FULL>(a, grid, st);
   } else {
-    if (g.stacked) launch_attend<DT, DP, false, true>(a, grid, st);
-    else launch_attend<DT, DP, false, false>(a, grid, st);
+    if (g.stacked) launch_attend<DT, DP, false, true, FULL>(a, grid, st);
+    else launch_attend<DT, DP, false, false, FULL>(a, grid, st);
   }
+}
+
+template <int DT, int DP>
+void launch(const AttnArgs& a, const Plan& g, hipStream_t st) {
+  // Heads that fill the padded size load their keys without a choice of lanes (one chunk of 50, 8 heads of 256, 816
+  // keys: 15.4 us for 16.3; 48 requests over 65537 keys: 61.5 for 64).
+  if (a.p.D == DP) launch_sweep<DT, DP, true>(a, g, st);
+  else launch_sweep<DT, DP, false>(a, g, st);
   const int64_t rows = part_rows(a.p);
   constexpr int ROUND = 4 * 64 / (DP / 4);  // parts that a wave has in flight
   if (g.parts > 8 * ROUND) launch_join<DT, DP, 16>(a, rows, st);

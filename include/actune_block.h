@@ -112,8 +112,7 @@ int actune_adapter_add(const actune_adapter_args* args, void* stream);
  * keys j < lengths[b]; causal: query t sees own keys j <= lengths[b] - T + t.
  * Lengths are clamped to [0, P] and [0, S]. A query that sees no key: out 0,
  * lse -inf. Keys and values that a query does not see may hold anything, NaN
- * included; the keys that it sees have to be finite where D is not 64, 128 or
- * 256 (an infinite one makes the query's result NaN).
+ * included.
  *
  * q: [B, T, Hq, D]; prefix_k, prefix_v: [G, P, Hkv, D]; k, v: [B, S, Hkv, D];
  * out: [B, T, Hq, D], dense; lse: f32 [B, T, Hq], dense, or NULL. bf16 or

@@ -171,3 +171,29 @@ def test_adapters_keep_to_their_rows_in_every_form(m, k, n, r):
     kept = (ids != 1) & (torch.arange(m, device=DEV) != 1)
     assert torch.equal(got[kept], want[kept])
     assert bool(got[ids == 1].isnan().any()) and bool(got[1].isnan().all())
+
+
+# every layout of the rows (32 or 128, a sequence's or a group's) at head sizes that fill no padded one, and at full ones
+@pytest.mark.parametrize("b,t,hq,hkv,d,p,s,causal", [
+    (1, 3, 4, 2, 8, 70, 5, True), (1, 50, 8, 1, 40, 300, 50, False), (2, 5, 8, 2, 80, 500, 17, True),
+    (1, 50, 8, 1, 200, 300, 50, False), (12, 3, 4, 4, 56, 2500, 40, True), (12, 3, 4, 4, 104, 2500, 40, True),
+    (12, 3, 4, 4, 136, 2500, 40, True), (40, 64, 4, 4, 24, 130, 70, True), (40, 64, 4, 4, 120, 130, 70, True),
+    (40, 64, 4, 4, 248, 130, 70, True), (130, 1, 8, 2, 48, 1500, 5, False), (130, 1, 8, 2, 88, 1500, 5, False),
+    (130, 1, 8, 1, 152, 1500, 70, False), (40, 64, 4, 4, 128, 130, 70, True), (130, 1, 8, 1, 256, 1500, 70, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_attention_keys_of_infinite_scores(b, t, hq, hkv, d, p, s, causal, dtype):
+    """A key that its queries see with a score of minus infinity counts nothing, one of plus infinity gives NaN, at every
+    head size: what stands for the columns past it is no part of the score."""
+    from actune_amd.kernels.attention import shared_prefix_attention
+    gen = block._gen(d + b)
+    q, pk, pv, k, v = block._attention_inputs(gen, b, t, hq, hkv, d, p, s, 1, dtype)
+    q[..., 0] = (q[..., 0].abs() + 1).to(dtype)
+    q[..., d - 1] = (q[..., d - 1].abs() + 1).to(dtype)
+    pk[:, ::3, :, 0] = -torch.inf
+    pk[:, 1::5, :, d - 1] = -torch.inf
+    k[:, 0::4, :, 0] = -torch.inf
+    got = block._check_attention(q, pk, pv, k, v, dtype, causal=causal)
+    pk[:, p // 2, 0, 0], pk[:, p // 2, 0, d - 1] = torch.inf, 0
+    bad = shared_prefix_attention(q, pk, pv, k, v, causal=causal)
+    share = hq // hkv
+    assert bool(bad[:, :, :share].isnan().all()) and torch.equal(bad[:, :, share:], got[:, :, share:])
