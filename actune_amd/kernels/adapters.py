@@ -104,7 +104,10 @@ def active_adapter_ids():
 class AdaptedLinear(torch.nn.Module):
     """A packed linear (any module with in_features and out_features) with L
     adapters of rank R beside it, in the dtype of the activations. Outside an
-    adapter_scope it is the linear alone."""
+    adapter_scope it is the linear alone. It stands in for the linear: what it
+    has no attribute of its own for (weight, active_backend, assignments, ..)
+    is the linear's, the call counters among it, and sibling and gated
+    launches (kernels.grouped) take it."""
 
     def __init__(self, base, a, b, scaling):
         super().__init__()
@@ -114,11 +117,35 @@ class AdaptedLinear(torch.nn.Module):
                              f"{list(a.shape)}, {list(b.shape)}")
         if tuple(scaling.shape) != (a.shape[0],) or scaling.dtype != torch.float32:
             raise ValueError("scaling must be one float32 for each adapter")
-        self.base = base
         self.in_features, self.out_features = base.in_features, base.out_features
         self.register_buffer("a", a.detach().contiguous())
         self.register_buffer("b", b.detach().contiguous())
         self.register_buffer("scaling", scaling.detach().contiguous())
+        self.base = base  # (behind the buffers: attributes are the base's from here on)
+
+    def __getattr__(self, name):
+        try:
+            return super().__getattr__(name)
+        except AttributeError:
+            if name == "base" or name.startswith("__"):  # (not set yet; python's own)
+                raise
+            return getattr(self.base, name)
+
+    @property
+    def calls(self):
+        return self.base.calls
+
+    @calls.setter
+    def calls(self, value):
+        self.base.calls = value
+
+    @property
+    def input_elements(self):
+        return self.base.input_elements
+
+    @input_elements.setter
+    def input_elements(self, value):
+        self.base.input_elements = value
 
     def adapt(self, y, x):
         """y (the linear's output on x, which this may write) with the scope's

@@ -23,6 +23,7 @@ import torch
 
 from .. import _native
 from ..precision import active_precision_profile
+from .adapters import AdaptedLinear, active_adapter_ids
 from .quantizers import weight_codes
 
 CONFIG_AUTO = _native.CONFIG_AUTO
@@ -279,6 +280,12 @@ def _zero_padded(linear, padded):
     return fc
 
 
+def _is_packed(module):
+    while isinstance(module, AdaptedLinear):
+        module = module.base
+    return isinstance(module, GroupedPaddedLinear)
+
+
 def _gate_kind(act_fn):
     """The gated quantizer's code for an activation whose torch form it
     reproduces (SiLU; GELU with the tanh approximation, Gemma's
@@ -304,7 +311,10 @@ def gated_down_forward(down, gate, up, act_fn):
     down's quantizer launch (actune_quantize_gated: one launch in place of
     three) and down runs on its codes; the output is bit-identical to the
     unfused calls and down's calls / input_elements advance as for one call.
-    Otherwise the unfused calls run."""
+    Otherwise the unfused calls run (also where down is an AdaptedLinear
+    inside an adapter_scope: its adapters read the product itself)."""
+    while isinstance(down, AdaptedLinear) and active_adapter_ids() is None:
+        down = down.base
     kind = _gate_kind(act_fn)
     backend = down.active_backend() if isinstance(down, GroupedPaddedLinear) else None
     scale = getattr(down, "input_scale", None)
@@ -338,7 +348,7 @@ def _inference_mlp(self, x):
     if torch.is_grad_enabled():
         return self._group64_original_forward(x)
     gate_proj, up_proj = self.gate_proj, self.up_proj
-    if isinstance(gate_proj, GroupedPaddedLinear) and isinstance(up_proj, GroupedPaddedLinear):
+    if _is_packed(gate_proj) and _is_packed(up_proj):
         gate, up = grouped_sibling_forward(x, [gate_proj, up_proj])
     else:
         gate, up = gate_proj(x), up_proj(x)
@@ -361,7 +371,8 @@ def reuse_mlp_temporary(model):
 def grouped_sibling_forward(x, modules):
     """Run GroupedPaddedLinear (or ResidentLinear) modules that read the same
     input x — sibling projections such as q/k/v or gate/up — and return their
-    outputs in order.
+    outputs in order. AdaptedLinears of such modules add their adapters behind
+    the launch.
 
     When every module's active backend has the same A, K, padding, bias
     dtype and input scale, all of them run in one actune_grouped_forward_multi
@@ -374,6 +385,9 @@ def grouped_sibling_forward(x, modules):
     modules = list(modules)
     if not modules:
         return []
+    if any(isinstance(m, AdaptedLinear) for m in modules):
+        outs = grouped_sibling_forward(x, [m.base if isinstance(m, AdaptedLinear) else m for m in modules])
+        return [m.adapt(y, x) if isinstance(m, AdaptedLinear) else y for m, y in zip(modules, outs)]
     backends = [m.active_backend() for m in modules]
     first, fb = modules[0], backends[0]
     scale = getattr(first, "input_scale", None)

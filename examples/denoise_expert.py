@@ -62,10 +62,9 @@ class Block(torch.nn.Module):
 
     def attend(self, x, prefix_k, prefix_v, prefix_mask):
         b, t, _ = x.shape
-        q, k, v = grouped_sibling_forward(x, [self.query.base, self.key, self.value])
-        q = self.query.adapt(q, x).view(b, t, HEADS, HEAD)
-        out = shared_prefix_attention(q, prefix_k, prefix_v, k.view(b, t, 1, HEAD), v.view(b, t, 1, HEAD),
-                                      prefix_mask=prefix_mask)
+        q, k, v = grouped_sibling_forward(x, [self.query, self.key, self.value])
+        out = shared_prefix_attention(q.view(b, t, HEADS, HEAD), prefix_k, prefix_v, k.view(b, t, 1, HEAD),
+                                      v.view(b, t, 1, HEAD), prefix_mask=prefix_mask)
         return self.output(out.view(b, t, HEADS * HEAD))
 
     def feed_forward(self, x):

@@ -1,12 +1,14 @@
 """The adapters where they meet the rest of the framework, on the GPU: graph
-replay under an adapter scope, codes that linears share."""
+replay under an adapter scope, codes that linears share, adapted linears in
+sibling and gated launches."""
 import pytest
 import torch
 
 from actune_amd import _block, _native
 from actune_amd.graph import GraphReplay
 from actune_amd.kernels.adapters import AdaptedLinear, adapter_add, adapter_scope
-from actune_amd.kernels.grouped import GroupedPaddedLinear, shared_activation_scope
+from actune_amd.kernels.grouped import (GroupedPaddedLinear, grouped_sibling_forward, reuse_mlp_temporary,
+                                        shared_activation_scope)
 from actune_amd.kernels.tokenwise import W4A8TritonLinear, shared_a8_cache_scope
 
 pytestmark = pytest.mark.gpu
@@ -93,3 +95,57 @@ def test_codes_of_a_written_tensor_are_not_used_again(mode, native, kind, monkey
             with torch.no_grad(), scope():
                 assert torch.equal(got, second(t.clone()))
             assert not torch.equal(got, stale)
+
+
+@pytest.mark.parametrize("m", [1, 50, 200])
+def test_adapted_siblings_equal_separate_calls(m):
+    """Sibling projections of which some carry adapters: one launch for the linears, the adapters behind it, in a scope
+    and outside; counters as for separate calls."""
+    torch.manual_seed(2)
+    with torch.inference_mode():
+        q, k, v = (_packed(1024, n) for n in (2048, 256, 256))
+        q, v = _adapted(q), _adapted(v, rank=40)
+        x = torch.randn(m, 1024, device=DEV, dtype=torch.bfloat16)
+        for ids in (None, torch.arange(m, device=DEV, dtype=torch.int32) % 4 - 1):
+            with adapter_scope(ids):
+                want = [layer(x) for layer in (q, k, v)]
+                before = [layer.calls for layer in (q, k, v)]
+                got = grouped_sibling_forward(x, [q, k, v])
+            assert all(torch.equal(g, w) for g, w in zip(got, want))
+            assert [layer.calls for layer in (q, k, v)] == [n + 1 for n in before]
+
+
+def test_an_adapted_mlp_keeps_its_launches(monkeypatch):
+    """A GemmaMLP whose projections all carry adapters: patched as unpatched, bit for bit, in a scope and outside, and
+    replayed; outside a scope gate and up share a launch and the product is formed in down's quantizer."""
+    from transformers import GemmaConfig
+    from transformers.models.gemma.modeling_gemma import GemmaMLP
+    torch.manual_seed(3)
+    cfg = GemmaConfig(hidden_size=1024, intermediate_size=4096, hidden_activation="gelu_pytorch_tanh")
+    mlp = GemmaMLP(cfg).to(device=DEV, dtype=torch.bfloat16)
+    with torch.inference_mode():
+        for name in ("gate_proj", "up_proj", "down_proj"):
+            linear = GroupedPaddedLinear(getattr(mlp, name), {"q11": "w4a8"}, "q11", {"w4a8": None})
+            setattr(mlp, name, _adapted(linear))
+        x = torch.randn(5, 10, 1024, device=DEV, dtype=torch.bfloat16)
+        scopes = (None, _ids(0, 1, -1, 2, 0), _ids(2, 2, 1, -1, -1))
+
+        def run(module, ids):
+            with adapter_scope(ids):
+                return module(x).clone()
+
+        want = [run(mlp, ids) for ids in scopes]
+        assert reuse_mlp_temporary(mlp) == 1
+        gated, multi = [], []
+        for name, seen in (("quantize_gated", gated), ("grouped_forward_multi", multi)):
+            call = getattr(_native, name)
+            monkeypatch.setattr(_native, name, lambda *a, _call=call, _seen=seen, **kw: (_seen.append(1), _call(*a, **kw))[1])
+        for ids, w in zip(scopes, want):
+            assert torch.equal(run(mlp, ids), w)
+        assert len(multi) == 3 and len(gated) == 1
+        replay = GraphReplay(mlp, {n: getattr(mlp, n) for n in ("gate_proj", "up_proj", "down_proj")}, shared_a8=True)
+        replay.enabled = True
+        for ids, w in (*zip(scopes, want), *zip(scopes, want)):
+            assert torch.equal(run(replay, ids), w)
+            torch.cuda.synchronize()
+        assert len(replay.graphs) == 2
