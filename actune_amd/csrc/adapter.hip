@@ -380,10 +380,12 @@ __global__ __launch_bounds__(64 * kWaves) void adapter_up(const AdapterArgs args
 // large ones (us, kernels alone, one launch against two, which wait for each
 // other as well): 64 tokens, 1024 to 1024, rank 16, 4.0 against 3.3 + 4.8; 50
 // tokens, 1024 to 2048, rank 32, 5.3 against 3.7 + 4.6; 12 tokens, 4096 to 4096,
-// rank 16, 7.4 against 3.4 + 5.6; beyond the rule 12 tokens, 4096 to 11008 (two
-// rounds of the chip), 11.9 against 3.3 + 5.9, and 4096 to 4096 at rank 64, 19
-// against 4.2 + 6.6. More steps of K under way: no change. RT: 16-row tiles of
-// the rank.
+// rank 16, 7.4 against 3.4 + 5.6. Whole calls along the rule's product of rounds of
+// the chip, rank and K, 12 tokens to 4096 columns: at 73728 (rank 16, K 4608) 7.7
+// against 10.4, at 98304 (K 6144) 9.3 against 11.0; at 131072 they meet: 11.4
+// against 11.7 (K 8192), 11.1 against 9.9 (rank 32, K 4096), 11.7 against 10.3
+// (rank 16, K 4096, 11008 columns: two rounds); at rank 64 19 against 11. More
+// steps of K under way: no change. RT: 16-row tiles of the rank.
 constexpr int kOneWaves = 8, kOneColumns = 64 * kOneWaves, kOneRank = 32;
 
 template <int DT, int RT>
@@ -528,7 +530,7 @@ Plan plan_of(int64_t M, int64_t N, int64_t K, int64_t R) {
   g.RP = (int)((R + 15) / 16) * 16;
   const int64_t rounds = (M * ((N + kOneColumns - 1) / kOneColumns) + kCus - 1) / kCus;
   // (a grid's y stays below 2^16)
-  g.one = M <= 64 && R <= kOneRank && rounds * g.RP * K <= 65536 && N <= kOneColumns * 65535;
+  g.one = M <= 64 && R <= kOneRank && rounds * g.RP * K <= 98304 && N <= kOneColumns * 65535;
   const int64_t steps = (K + 255) / 256, blocks = (N + 255) / 256;
   auto groups = [&](int64_t t) { return (M + t - 1) / t; };
   g.down_tokens = M <= 64 ? 1 : groups(16 * kDownTiles) * (steps < 16 ? steps : 16) < 2 * kCus ? 16 : 16 * kDownTiles;

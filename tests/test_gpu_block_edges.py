@@ -86,8 +86,9 @@ def test_attention_batches_past_a_dispatch(b, heads, p, s, g):
         block._near(lse[rows, 0], torch.logsumexp(scores, 1), 1e-4, first)
 
 
-# one launch; two: a token a workgroup, tiles of 16, of 64 and (rank above 64) of 32 tokens
-ADAPTER_FORMS = [(5, 512, 96, 16), (5, 512, 96, 40), (5, 512, 96, 100), (70, 512, 96, 16), (70, 520, 100, 128),
+# one launch, and the largest K of one with 16 ranks; two: a token a workgroup, tiles of 16, of 64 and (rank above 64) of
+# 32 tokens
+ADAPTER_FORMS = [(5, 512, 96, 16), (12, 6143, 1030, 16), (12, 6160, 1030, 16), (5, 512, 96, 40), (5, 512, 96, 100), (70, 512, 96, 16), (70, 520, 100, 128),
                  (2100, 8200, 2100, 16), (2100, 8200, 2100, 64), (2100, 8200, 1030, 128)]
 
 
