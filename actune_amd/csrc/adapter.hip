@@ -11,7 +11,8 @@
 // of its tokens; an adapter's matrix is read straight from memory, 16 bytes a
 // lane, as the MFMA's operand, once for all its tiles with a token of that id,
 // and the columns of the tokens that name it are kept. Tokens of one request
-// stand side by side, so that a workgroup meets one or two ids. Rows of
+// stand side by side, so that a workgroup meets one or two ids where requests
+// have tens of tokens; it goes through more of them one after the other. Rows of
 // different ids never meet in a sum: one adapter's infinities stay with its
 // requests.
 //
@@ -19,9 +20,11 @@
 // and the next step's operands are requested before this one's products. 8192
 // tokens of 8 requests, 4096 to 11008 columns, rank 64: 26 us down (67 MB of x,
 // 2.5 TB/s: its wait is for the operands of A beside them, 35 us with 32 tokens
-// a workgroup) and 96 us up (361 MB of y and out, 3.8 TB/s; a copy of as much
+// a workgroup) and 98 us up (361 MB of y and out, 3.7 TB/s; a copy of as much
 // takes 75). 12 tokens with an adapter each, 4096 to 4096, rank 16: one launch of
-// 7.4 us.
+// 7.4 us. Single tokens with an adapter each are slow above 64, where a workgroup
+// has 16 of them: 64, 65, 128 and 256 of them, same sizes, take 10, 35, 49 and 51
+// us a call.
 #include <climits>
 
 #include "block.hpp"

@@ -31,16 +31,27 @@
 //     busy 39 percent of the cycles, the vector units issue in 45: a wave's tile
 //     goes through products, exponentials and products, and the two waves a SIMD
 //     overlap only in part.
-//   32 chunks of 50, 8 heads of 256 over one, 768 keys seen of 968 and 50: 34.8
-//     + 7.2 us, 0.31 PFLOP/s. Each workgroup sweeps 9 tiles (20 us); the rest is
-//     its start, 26 MB of parts, and reading them again.
-//   24 requests, 32 heads of 128, 4096 keys and 160: 32 + 4.7 us for 114 MB.
+//   32 chunks of 50, 8 heads of 256 over one, 768 keys seen of 968 and 50: 34.4
+//     + 7.0 us, 0.31 PFLOP/s. Each workgroup sweeps 9 tiles (20 us), those that
+//     the mask empties among them; the rest is its start, 26 MB of parts, and
+//     reading them again.
+//   24 requests, 32 heads of 128, 4096 keys and 160: 31 + 4.7 us for 114 MB.
 //     Bound by the own keys' items, whose loads are a few tiles deep.
-//   48 requests, 8 heads of 256 over one, 65537 keys and 300 (f16): 55 + 8.2 us,
-//     78 MB and 26 GFLOP: 3.2 us a tile of 64 keys for 2.4 where the keys are in
-//     cache, the wait for memory one tile ahead.
+//   48 requests, 8 heads of 256 over one, 65537 keys and 300 (f16): 53 + 8.0 us,
+//     78 MB and 26 GFLOP. Bound by its cut: 159 workgroups sweep 20 tiles of 64
+//     keys each, 2.3 us a tile, beside 96 with two or three tiles of own keys
+//     (own keys in one item each leave room for 240 with 15 tiles: 45 + 9.0).
 //   one request, 8 heads of 128 read by 32, 65536 keys: 45 us, 268 MB, 5.9 TB/s.
-//   one chunk of 50, 816 keys: 12.4 + 4.2 us, most of it two launches' latency.
+//   one chunk of 50, 816 keys: 12.1 + 4.0 us, most of it two launches' latency.
+//
+// The probabilities are rounded to the operands' type for the second product,
+// their sum is not. That is where the outputs' error comes from beside their own
+// rounding: 0.0022 of the 2-norm in bf16 (f32 probabilities: 0.0017), 0.00028 in
+// f16 (0.00021), where many keys count. A second 16-bit part of them takes it
+// away for half as many products again: 242 us for the 190 of the prompts, 39.2
+// for 37.5 a call of the 24 requests, 15.9 for 15.4 of the one chunk; the wave
+// pairs have no LDS for it. One part in every form, so that the precision does
+// not depend on the layout.
 #include <climits>
 #include <cmath>
 
@@ -1216,6 +1227,8 @@ bool sizes_ok(const actune_prefix_attention_args& p) {
 // (measured alone and on a full chip: 128 rows of heads of 256 take 8.9 us with
 // one tile and 14.8 with four, of 128 6.8 and 10.0; 32 rows 8.0 and 13.0, 5.8
 // and 8.2 with tiles of 64 and 128 keys), and how many the chip holds at a time.
+// Two workgroups a CU that are at work throughout slow each other: eight prompts
+// of 512 with heads of 128 take 2.2 us a tile, 190 us where these give 134.
 struct Cost {
   double fixed, tile;
   int slots;
@@ -1246,7 +1259,8 @@ double cut_plan(const actune_prefix_attention_args& p, const Sizes& z, bool big,
   if (stacked && p.S > 0) {
     g.own_tiles = (int)tiles(z.rows, tr);
     own = p.B * p.Hkv * g.own_tiles;
-    // own keys: an item as long as a few of the main items' tiles; they fill what the chip has left
+    // own keys: an item as long as a few of the main items' tiles; they fill what the chip has left, before the main
+    // items are cut for the rest
     const int64_t want = own >= c.slots ? 1 : (c.slots + own - 1) / own, most = (g.own_cap + 3) / 4;
     g.own_splits = (int)(want < most ? want : most);
     if (g.own_splits < 1) g.own_splits = 1;
@@ -1287,7 +1301,8 @@ double cut_plan(const actune_prefix_attention_args& p, const Sizes& z, bool big,
 //   48 tokens, 8 heads of 256, 65537 keys       -         109        357           53
 //   8 prompts of 512, 32 heads of 128         381           -        190          260
 // Cuts of the first: 18.9 with 4, 15.8 with 8, 16.6 with 14; of the second, one
-// part 44 and two 40.7; of the fourth 77 with 34, 53 with 69, 61 with 85.
+// part 44 and two 40.7; of the fourth 77 with 34, 53 with 69, 61 with 85 (with
+// 53, which the own keys' two splits leave: 61).
 // 32-bit counts hold for every size that sizes_ok takes: items are at most rows
 // plus a bounded number of splits of them.
 Plan plan_of(const actune_prefix_attention_args& p) {

@@ -51,6 +51,8 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, *, prefix_len
     sum, f32 [B, T, Hq], by which the result can be joined with attention over
     further keys. A query that sees no key gets 0 and -inf. What keys and
     values hold that a query does not see does not matter to it, NaN included.
+    Scores, sums and the softmax's statistics are f32; its probabilities are
+    rounded to q's type for the product with the values.
     """
     single = isinstance(prefix_k, torch.Tensor) and prefix_k.dim() == 3 and isinstance(prefix_v, torch.Tensor)
     if single:

@@ -112,7 +112,8 @@ int actune_adapter_add(const actune_adapter_args* args, void* stream);
  * keys j < lengths[b]; causal: query t sees own keys j <= lengths[b] - T + t.
  * Lengths are clamped to [0, P] and [0, S]. A query that sees no key: out 0,
  * lse -inf. Keys and values that a query does not see may hold anything, NaN
- * included.
+ * included. Scores, statistics and sums are f32; the probabilities are rounded
+ * to the call's type for their product with the values.
  *
  * q: [B, T, Hq, D]; prefix_k, prefix_v: [G, P, Hkv, D]; k, v: [B, S, Hkv, D];
  * out: [B, T, Hq, D], dense; lse: f32 [B, T, Hq], dense, or NULL. bf16 or
